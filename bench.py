@@ -701,6 +701,34 @@ def planned_shards_figure(ctx):
     return fig
 
 
+class SetUpStep:
+    """One step of setting up a comparator: `make()` on the ranks in `who` (root / others / all), then every rank hears
+    whether it worked everywhere.  refused = None, or the first rank's reason; the step behind a refused one makes nothing
+    and hands the reason on.  No rank leaves on its own: the others would wait for it in their next collective."""
+
+    def __init__(self, ctx, who, make, after=None):
+        dist, rank, world = ctx["dist"], ctx["rank"], ctx["world"]
+        self.piece, self.refused = None, after.refused if after is not None else None
+        if self.refused:
+            return
+        why = None
+        if who == "all" or (who == "root") == (rank == 0):
+            try:
+                self.piece = make()
+            except Exception as e:   # noqa: BLE001  (e.g. IPC not offered by this host: said in the line, nothing measured)
+                why = str(e) or type(e).__name__
+        whys = [why]
+        if world > 1:
+            whys = [None] * world
+            dist.all_gather_object(whys, why)
+        self.refused = next((w for w in whys if w), None)
+
+    def close(self):
+        if self.piece is not None:
+            self.piece.close()
+            self.piece = None
+
+
 def direct_gather_figure(ctx):
     """N > 1, separate key: the direct-write comparator of the gatherv.  Rank 0 exports its result
     buffer (rsp_shared_result_alloc: hipIpcGetMemHandle), the other rank processes map it, and every rank's kernels take
@@ -709,29 +737,20 @@ def direct_gather_figure(ctx):
     torch, dist, capi = ctx["torch"], ctx["dist"], ctx["capi"]
     args, world, rank = ctx["args"], ctx["world"], ctx["rank"]
     ncol, displs, s_main = ctx["ncol"], ctx["displs"], ctx["s_main"]
-    note = None
-    try:
-        box = [None, None]
-        if rank == 0:
-            shared = capi.SharedResult(ncol)
-            box = [shared.handle, f"/rsp_bench_{os.getpid()}"]
-        if world > 1:
-            dist.broadcast_object_list(box, src=0)
-        if rank != 0:
-            shared = capi.SharedResult(ncol, handle=box[0])
-        barrier = capi.HostBarrier(box[1], world, rank)
-    except Exception as e:                      # e.g. IPC not offered by this host: say so, measure nothing
-        note = f"not measured: {e}"[:160]
-        ok = torch.tensor([0.0], device=ctx["stat_dev"])
-    else:
-        ok = torch.tensor([1.0], device=ctx["stat_dev"])
+    shared = SetUpStep(ctx, "root", lambda: capi.SharedResult(ncol))
+    box = [None if shared.refused else shared.piece.handle, f"/rsp_bench_{os.getpid()}"] if rank == 0 else [None, None]
     if world > 1:
-        dist.all_reduce(ok, op=dist.ReduceOp.MIN)
-    if float(ok[0]) == 0.0:
-        notes = [None] * world
+        dist.broadcast_object_list(box, src=0)
+    mapped = SetUpStep(ctx, "others", lambda: capi.SharedResult(ncol, handle=box[0]), after=shared)
+    barrier = SetUpStep(ctx, "all", lambda: capi.HostBarrier(box[1], world, rank), after=mapped)
+    if barrier.refused:
+        barrier.close()
+        mapped.close()
         if world > 1:
-            dist.all_gather_object(notes, note)
-        return {"value": None, "note": ([n for n in notes if n] or [note])[0]} if rank == 0 else None
+            dist.barrier()                        # nobody has the root's buffer mapped any more
+        shared.close()
+        return {"value": None, "note": f"not measured: {barrier.refused}"[:160]} if rank == 0 else None
+    shared, barrier = (shared if rank == 0 else mapped).piece, barrier.piece
 
     class Out:                                   # what the prepared launcher needs of an output tensor
         def __init__(self, ptr):
@@ -864,33 +883,17 @@ def host_gather_figure(ctx):
     torch, dist, capi = ctx["torch"], ctx["dist"], ctx["capi"]
     args, world, rank = ctx["args"], ctx["world"], ctx["rank"]
     ncol, displs, s_main, shard = ctx["ncol"], ctx["displs"], ctx["s_main"], ctx["shard"]
-    note, vec, barrier = None, None, None
-    try:
-        box = [None]
-        if rank == 0:
-            box = [f"/rsp_bench_host_{os.getpid()}"]
-        if world > 1:
-            dist.broadcast_object_list(box, src=0)
-        if rank == 0:
-            vec = capi.SharedHostVector(box[0], ncol, create=True)
-        if world > 1:
-            dist.barrier()
-        if rank != 0:
-            vec = capi.SharedHostVector(box[0], ncol, create=False)
-        barrier = capi.HostBarrier(box[0] + "_b", world, rank)
-        ok = torch.tensor([1.0], device=ctx["stat_dev"])
-    except Exception as e:   # noqa: BLE001
-        note = f"not measured: {e}"[:160]
-        ok = torch.tensor([0.0], device=ctx["stat_dev"])
+    box = [f"/rsp_bench_host_{os.getpid()}" if rank == 0 else None]
     if world > 1:
-        dist.all_reduce(ok, op=dist.ReduceOp.MIN)
-    if float(ok[0]) == 0.0:
-        notes = [None] * world
-        if world > 1:
-            dist.all_gather_object(notes, note)
-        if vec is not None:
-            vec.close()
-        return {"value": None, "note": ([n for n in notes if n] or [note])[0]} if rank == 0 else None
+        dist.broadcast_object_list(box, src=0)
+    created = SetUpStep(ctx, "root", lambda: capi.SharedHostVector(box[0], ncol, create=True))
+    opened = SetUpStep(ctx, "others", lambda: capi.SharedHostVector(box[0], ncol, create=False), after=created)
+    barrier = SetUpStep(ctx, "all", lambda: capi.HostBarrier(box[0] + "_b", world, rank), after=opened)
+    if barrier.refused:
+        for made in (barrier, opened, created):
+            made.close()
+        return {"value": None, "note": f"not measured: {barrier.refused}"[:160]} if rank == 0 else None
+    vec, barrier = (created if rank == 0 else opened).piece, barrier.piece
     out = torch.empty(max(shard.ncol, 1), dtype=torch.float64, device=ctx["dev"])[:shard.ncol]
     launches = [capi.prepared_column_sums(xk, ctx["pt"], out, ctx["ws_main"], stream=s_main) for xk in ctx["xs"]]
     n = [0]
