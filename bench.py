@@ -101,8 +101,8 @@ GLOSSARY = {
     "direct_gather": "N > 1: every rank's kernels store into rank 0's result buffer (mapped with hipIpcOpenMemHandle) at the "
                      "rank's displacement; per call: launch, wait for the own stream, cross a shared-memory barrier; "
                      "NOT the protocol of `value`",
-    "host_gather": "N > 1: every rank copies its slice (hipMemcpyAsync behind its kernels) over its own host link into ONE page-locked "
-                   "vector in POSIX shared memory that all rank processes map; per call: launch, the copy, wait for the own stream, "
+    "host_gather": "N > 1: every rank copies its slice (hipMemcpyAsync behind its kernels) over its own host link into ONE vector "
+                   "in POSIX shared memory (pageable) that all rank processes map; per call: launch, the copy, wait for the own stream, "
                    "cross a shared-memory barrier -- the root then holds the whole vector in HOST memory; NOT the protocol of `value`",
     "config.peer_probe": "what the throw-away child processes saw before direct_gather was allowed between different devices: "
                          "passed | same device | no peer access | failed: ...",
@@ -213,7 +213,7 @@ def parse_args(argv=None):
                          "takes a throw-away process down, not the job (config.peer_probe says what it saw)")
     ap.add_argument("--host-gather", default="auto", choices=["auto", "on", "off"],
                     help="N > 1: the separate host_gather figure (SURVEY.md section 5's other comparator: every rank copies its slice "
-                         "over its own host link into ONE page-locked vector in shared memory; per call: kernels, the copy, a wait "
+                         "over its own host link into ONE vector in shared memory; per call: kernels, the copy, a wait "
                          "for the own stream, a host barrier).  auto = on")
     ap.add_argument("--peer-probe", nargs=2, type=int, metavar=("OWNER", "WRITER"), help=argparse.SUPPRESS)
     ap.add_argument("--peer-probe-writer", nargs=2, metavar=("HANDLE_HEX", "WRITER"), help=argparse.SUPPRESS)
@@ -877,9 +877,10 @@ def run_peer_probe(owner, writer, timeout_s=150, command=None):
 
 
 def host_gather_figure(ctx):
-    """N > 1, separate key: SURVEY.md section 5's other comparator -- per-GPU D2H into disjoint slices of ONE pinned buffer.
-    The buffer lives in POSIX shared memory, every rank maps and page-locks it; per call a rank launches its kernels, copies
-    its slice behind them (its own host link), waits for its stream and crosses a host barrier.  Never `value`."""
+    """N > 1, separate key: the other comparator -- per-GPU D2H into disjoint slices of ONE host buffer.  The buffer lives in
+    POSIX shared memory that every rank maps (pageable: locking pages that exist already is not offered everywhere); per call
+    a rank launches its kernels, copies its slice behind them (its own host link), waits for its stream and crosses a host
+    barrier.  Never `value`."""
     torch, dist, capi = ctx["torch"], ctx["dist"], ctx["capi"]
     args, world, rank = ctx["args"], ctx["world"], ctx["rank"]
     ncol, displs, s_main, shard = ctx["ncol"], ctx["displs"], ctx["s_main"], ctx["shard"]

@@ -976,8 +976,8 @@ class SharedResult:
 
 
 class SharedHostVector:
-    """n doubles in POSIX shared memory, mapped and page-locked in this process (rsp_shared_host_open): the rank processes'
-    copy engines write their slices into it, the root reads the whole (`array`)."""
+    """n doubles in POSIX shared memory, mapped in this process (rsp_shared_host_open; ordinary memory, not page-locked): the
+    rank processes copy their slices into it, the root reads the whole (`array`)."""
 
     def __init__(self, name: str, n: int, create: bool):
         self.name, self.n, self.bytes, self.create = name, int(n), max(8, 8 * int(n)), bool(create)
@@ -987,7 +987,7 @@ class SharedHostVector:
         self.array = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_double)), shape=(max(self.n, 1),))[:self.n]
 
     def copy_from_device(self, src_t, offset: int, stream=None) -> None:
-        """enqueue: src_t (float64, device) -> vector[offset : offset + len] on `stream`"""
+        """src_t (float64, device) -> vector[offset : offset + len] on `stream`; there once `stream` has been waited for"""
         _check(load().rsp_copy_to_host_async(src_t.data_ptr(), ctypes.c_void_p(self.ptr + 8 * int(offset)), int(src_t.numel()),
                                              _stream_ptr(stream)))
 

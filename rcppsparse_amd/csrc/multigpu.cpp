@@ -1389,10 +1389,12 @@ int rsp_shared_result_close(void* d_ptr, int owner) {
     return RSP_OK;
 }
 
-// ---- host-memory gather: one page-locked vector shared by the rank processes -------------------------------------
-// SURVEY.md section 5's other comparator: "per-GPU D2H into disjoint slices of one pinned buffer".  The vector lives in
-// POSIX shared memory; every rank maps it and page-locks ITS mapping (hipHostRegister), so its copy engine writes the
-// rank's slice straight into memory the root process reads -- over the rank's own host link, no xGMI hop, no RCCL.
+// ---- host-memory gather: one vector in memory shared by the rank processes ---------------------------------------
+// The comparator "per-GPU D2H into disjoint slices of one buffer".  The vector lives in POSIX shared memory that every rank
+// maps, and each rank copies its slice into its mapping over its own host link: no xGMI hop, no RCCL.  The mapping is
+// ordinary memory: locking pages that already exist (hipHostRegister) is refused by some hosts, and the error such a
+// refusal leaves can come back from a later call; locked memory has to be ALLOCATED locked, which memory shared between
+// processes cannot be.  The runtime's copy into pageable memory goes through its own locked buffers.
 // After the ranks' stream waits and one host barrier the root holds the complete vector in HOST memory (where an R
 // NumericVector has to end up anyway).
 int rsp_shared_host_open(const char* name, size_t bytes, int create, void** host_ptr) {
@@ -1425,13 +1427,6 @@ int rsp_shared_host_open(const char* name, size_t bytes, int create, void** host
     void* m = mmap(nullptr, mapped, PROT_READ | PROT_WRITE, MAP_SHARED | MAP_POPULATE, fd, 0);
     close(fd);
     if (m == MAP_FAILED) return fail(RSP_ERR_ALLOC, "mmap of %s failed", name);
-    const hipError_t e = hipHostRegister(m, mapped, hipHostRegisterPortable | hipHostRegisterMapped);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        munmap(m, mapped);
-        if (create) (void)shm_unlink(name);
-        return fail(RSP_ERR_HIP, "hipHostRegister of the shared vector: %s", hipGetErrorString(e));
-    }
     *host_ptr = m;
     return RSP_OK;
 }
@@ -1439,14 +1434,13 @@ int rsp_shared_host_open(const char* name, size_t bytes, int create, void** host
 int rsp_shared_host_close(void* host_ptr, size_t bytes, const char* unlink_name) {
     if (!host_ptr) return RSP_OK;
     const size_t mapped = (bytes + 4095) & ~(size_t)4095;
-    const hipError_t e = hipHostUnregister(host_ptr);
-    if (e != hipSuccess) (void)hipGetLastError();
     munmap(host_ptr, mapped);
     if (unlink_name) (void)shm_unlink(unlink_name);
     return RSP_OK;
 }
 
-// enqueue only: n doubles from device memory into (page-locked) host memory on `stream`
+// n doubles from device memory into host memory on `stream`: enqueue only where the destination is page-locked, else the
+// runtime may hold the caller until the slice has arrived; complete, either way, when `stream` is
 int rsp_copy_to_host_async(const double* d_src, double* host_dst, int64_t n, void* stream) {
     if (n < 0 || (n > 0 && (!d_src || !host_dst))) return fail(RSP_ERR_BAD_ARG, "bad argument to rsp_copy_to_host_async");
     if (n == 0) return RSP_OK;
